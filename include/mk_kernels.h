@@ -390,7 +390,8 @@ int mk_merge_heads_bf16(const void* o, void* out, int64_t B, int64_t H, int64_t 
  * reference function corresponds (its transformer benchmark,
  * benchmarks/vs_cpu.py:603-626, has whole sequences of one length and no
  * cache).  Strides are in elements, must be >= 0 and keep every head's start
- * aligned as stated; dimensions within a head are contiguous.  Values that
+ * aligned as stated; dimensions within a head are contiguous, and an output's
+ * heads must not share memory (MK_EINVAL).  Values that
  * live in device memory (positions, slots, block table entries, lengths,
  * offsets) are checked by the kernels, which never read or write outside the
  * sizes given: what a wrong value gives is stated per call.

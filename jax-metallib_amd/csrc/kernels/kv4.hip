@@ -310,6 +310,9 @@ extern "C" int mk_kv4_read(const mk_kv4_cache* cache, int dtype, void* k, void* 
   const int rc = rows_args(&a, cache, k, v, strides, slots, T, dtype == MK_DT_F32 ? 4 : 2, fn);
   if (rc != MK_OK) return rc;
   if (T == 0) return MK_OK;
+  for (int i = 0; i < 2; ++i)
+    if (!mkc::runs_apart({T, a.c.heads, 1}, {a.tok[i], a.head[i], 0}, cache->dim))
+      return mkc::fail(MK_EINVAL, "%s: an output's heads share memory", fn);
   a.in[0] = a.in[1] = nullptr;
   a.out[0] = k;
   a.out[1] = v;

@@ -674,6 +674,8 @@ extern "C" int mk_attention_kv4_bf16(const void* q, const mk_kv4_cache* cache, c
     (i < 3 ? a.q_strides : a.out_strides)[i % 3] = st;
   }
   if (((uintptr_t)q | (uintptr_t)out) % 16) return mkc::fail(MK_EINVAL, "%s: q and out must be 16-byte aligned", fn);
+  if (!mkc::runs_apart(dims, a.out_strides, cache->dim))
+    return mkc::fail(MK_EINVAL, "%s: the heads of out share memory", fn);
   a.q = static_cast<const uint16_t*>(q);
   a.out = static_cast<uint16_t*>(out);
   a.table = block_table;

@@ -516,6 +516,8 @@ extern "C" int mk_attention_packed_bf16(const void* q, const void* k, const void
   }
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16)
     return mkc::fail(MK_EINVAL, "%s: q, k, v and out must be 16-byte aligned", fn);
+  if (!mkc::runs_apart({Tq, Hq, 1}, {st8[6], st8[7], 0}, D))
+    return mkc::fail(MK_EINVAL, "%s: the heads of out share memory", fn);
   mk::PackedArgs a;
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);

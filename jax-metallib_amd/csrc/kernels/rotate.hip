@@ -234,6 +234,8 @@ extern "C" int mk_qk_norm_rope(int dtype, const void* q, const void* k, void* q_
   }
   if (bits % step || odd % 4 || ((uintptr_t)cos_table | (uintptr_t)sin_table) % 16)
     return mkc::fail(MK_EINVAL, "%s: heads must start at multiples of 4 elements, tables at 16 bytes", fn);
+  if (!mkc::runs_apart({T, Hq, 1}, {sd[4], sd[5], 0}, D) || !mkc::runs_apart({T, Hkv, 1}, {sd[6], sd[7], 0}, D))
+    return mkc::fail(MK_EINVAL, "%s: an output's heads share memory", fn);
   mk::RotateArgs a;
   a.in[0] = q; a.in[1] = k;
   a.out[0] = q_out; a.out[1] = k_out;

@@ -503,8 +503,9 @@ def _launch(device, call):
 
 
 def _strides(t, name, dtypes, shape, device, written=False):
-    """The strides of a tensor on the device whose last dimension is dense and
-    whose elements, if it is written, do not share memory."""
+    """The strides of a tensor on the device whose last dimension is dense and,
+    if it is written, has no stride of 0 (of other strides the C entries find
+    heads that share memory)."""
     st = t.stride()
     if t.get_device() == device.index and t.dtype in dtypes and t.shape == shape and st[-1] == 1 and \
             not (written and 0 in st) and t.is_cuda:
