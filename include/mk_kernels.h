@@ -451,7 +451,10 @@ int mk_merge_heads_bf16(const void* o, void* out, int64_t B, int64_t H, int64_t 
  *   Offsets are taken in 0 .. Tq (Tk).  D is 64 or 128.
  * Both attentions may write over q (out = q).  They keep scores, maximum, sum
  * and output in f32, the sum of p v (p <= 1) undivided until the end: it must
- * stay in the f32 range.  scale must be positive and finite.
+ * stay in the f32 range, and with the 4-bit cache so must the sum of p and the
+ * largest |v| of each key's group (there scales below 2^-113 lose bits, as p
+ * times the scale, p below 2^-5, is rounded to bf16).  scale must be positive
+ * and finite.
  * ---------------------------------------------------------------------- */
 enum { MK_ROPE_HALF = 0, MK_ROPE_INTERLEAVED = 1 };
 

@@ -64,6 +64,10 @@ struct Kv4AttnArgs {
 
 constexpr int kKaTile = 64;  // keys per tile
 constexpr float kKaSlack = 8.f;  // log2 units
+// p is held below 2^-5, so that the offsets (128 + z <= 143 steps of a scale,
+// where the largest value of a group has 7 or more) cannot pass the f32 range
+// before the sum of p times those largest values does.
+constexpr float kKaLift = kKaSlack + 5.f;
 constexpr int kKaWaves = 4;  // per workgroup
 constexpr int kKaLog = 11;   // log2 of the waves that share the work
 
@@ -393,7 +397,7 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_kernel(Kv4AttnArgs a) {
         for (int e = 0; e < 4; ++e) mt = fmaxf(mt, s[tt][e]);
       mt = quad_max(mt);
       // m follows the maximum only when some row has passed it by kKaSlack, and
-      // p counts from m + kKaSlack, so it stays below 1 and most tiles rescale
+      // p counts from m + kKaLift, so it stays below 2^-5 and most tiles rescale
       // nothing.
       const float mn = fmaxf(m, mt * a.scale_log2);  // the scale is positive
       if (!__all(mn <= m + kKaSlack)) {
@@ -403,7 +407,7 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_kernel(Kv4AttnArgs a) {
 #pragma unroll
         for (int n = 0; n < NB; ++n) o[n] *= alpha;
       }
-      const float ref = m == -INFINITY ? 0.f : m + kKaSlack;
+      const float ref = m == -INFINITY ? 0.f : m + kKaLift;
       float ps = 0.f;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)

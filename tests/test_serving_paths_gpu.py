@@ -3,11 +3,15 @@ and lists: strided outputs, batches that fill the card, far slots, values at the
 ends of the range.  Oracles are in float64, tolerances are sums of the
 documented roundings: half a step of bf16 is 2^-8 of the value, of f32 2^-24."""
 
+import math
+
 import numpy as np
 import pytest
 
 from _gpu import torch
-from test_serving_ops_gpu import DEV, _cu, _ints, _ops, _rand, _up
+from oracle import serving
+from oracle.bf16 import round_bf16
+from test_serving_ops_gpu import DEV, _attention_bound, _check, _cu, _down, _ints, _ops, _rand, _up
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +51,34 @@ def test_outputs_whose_heads_share_memory_are_refused():
     for call, (w, w2) in zip(calls(_window((T, H, D), (128, 832, 1)), _window((T, H, D), (832, 128, 1))), want):
         out, out2 = call()
         assert torch.equal(out.reshape(w.shape), w) and torch.equal(out2, w2)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_kv4_largest_values(D):
+    """Values as large as they may be, most of them with the weight 1: the sum
+    of p and the largest |v| of each key's group, p <= 1, stays in the f32 range
+    for 400 keys up to 2^119 (400 < 2^8.65; the format keeps at most 16 / 15
+    of a value, 2^0.1).  The waves' runs have two or three tiles, and the running
+    maximum may lag by 2^8 (the first tile's scores are 0, all others'
+    7.9 .. 8 in units of log 2), so p reaches 1 within a tile."""
+    ops = _ops()
+    n, H, B, page = 400, 8, 96, 16
+    rng = np.random.default_rng(2)
+    q = np.zeros((1, H, D), np.float32)
+    q[:, :, 0] = 1.0
+    k = np.zeros((n, H, D), np.float32)
+    k[64:, :, 0] = 5.53
+    v = round_bf16(rng.choice([-1.0, 1.0], (n, H, D)).astype(np.float32) * 2.0 ** 119)
+    k = round_bf16(k)
+    kq = serving.kv4_values(*serving.kv4(k))
+    assert (kq[64:, :, 0] * math.log2(math.e) < 8).all() and (kq[64:, :, 0] * math.log2(math.e) > 7.9).all()
+    vq = serving.kv4_values(*serving.kv4(v)) / 2.0 ** 119
+    assert n * np.abs(vq).max() * 2.0 ** 119 < 2.0 ** 128
+    cache = ops.KV4Cache(n // page, H, page, D, device=DEV)
+    ops.kv4_append(cache, _up(k), _up(v), _ints(np.arange(n), torch.int64))
+    table = np.tile(np.arange(n // page), (B, 1))
+    y = ops.attention_kv4(_up(np.tile(q, (B, 1, 1, 1))), cache, _ints(table), _ints(np.full(B, n)), 1.0)
+    got = _down(y) / 2.0 ** 119
+    ref, mag = serving.attention(q, kq, vq, 1.0, np.ones((1, n), bool))
+    bound = _attention_bound(ref, mag, q, k, 1.0, n, kv4=True)
+    _check(got, np.tile(ref, (B, 1, 1, 1)), np.tile(bound, (B, 1, 1, 1)), f"kv4 largest values {D}")
