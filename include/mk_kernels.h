@@ -449,7 +449,8 @@ int mk_merge_heads_bf16(const void* o, void* out, int64_t B, int64_t H, int64_t 
  *   gives zeros.  A NaN or infinity in v gives NaN or an infinity in the rows
  *   that see it only.  Rows of out that belong to no sequence are not written.
  *   Offsets are taken in 0 .. Tq (Tk).  D is 64 or 128.
- * Both attentions may write over q (out = q).  They keep scores, maximum, sum
+ * Both attentions may write over q (out = q).  A query that sees keys, all with
+ * the score -infinity, gives NaN.  They keep scores, maximum, sum
  * and output in f32, the sum of p v (p <= 1) undivided until the end: it must
  * stay in the f32 range, and with the 4-bit cache so must the sum of p and the
  * largest |v| of each key's group (there scales below 2^-113 lose bits, as p

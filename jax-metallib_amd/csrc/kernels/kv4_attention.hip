@@ -140,6 +140,21 @@ __device__ __forceinline__ int ka_wave_of(int x, int all) {
   return x;
 }
 
+// Whether one of the first `lim` keys of sequence b lies in a page the cache
+// has.
+__device__ __forceinline__ bool ka_sees(const Kv4AttnArgs& a, int b, int lim) {
+  const int32_t* table = a.table + (int64_t)b * a.width;
+  for (int c = 0; (int64_t)c * a.c.page < lim; ++c)
+    if (table[c] >= 0 && table[c] < a.c.pages) return true;
+  return false;
+}
+
+// What a row of the sum `sum` is multiplied with at the end: no key seen gives
+// zeros, only scores of -infinity NaN.
+__device__ __forceinline__ float ka_inverse(const Kv4AttnArgs& a, float sum, int b, int lim) {
+  return sum == 0.f && !ka_sees(a, b, lim) ? 0.f : 1.0f / sum;
+}
+
 // 8 numbers of 4 bits as the bf16 128 + n, in the order 0 4 1 5 2 6 3 7.  The
 // mask M = 0x000f000f comes in a vector register: v_and_or_b32 takes one
 // constant only.
@@ -461,7 +476,7 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_kernel(Kv4AttnArgs a) {
     // The end of an item that this wave has to itself, or a part of one.
     if (!joined && l16 < left) {
       if (whole) {
-        const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
+        const float inv = ka_inverse(a, lsum, b, lim);
         uint16_t* out = a.out + b * a.out_strides[0] + qi * a.out_strides[1] + qh * a.out_strides[2] + 4 * g;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -481,6 +496,7 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_kernel(Kv4AttnArgs a) {
     }
   }
   if (!joined) return;  // the same for all four waves
+  const int jlen = lens.keys(a, jb);
 
   // Join the waves: each leaves its rows in its own stages.
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -511,8 +527,8 @@ __global__ __launch_bounds__(256, 2) void attention_kv4_kernel(Kv4AttnArgs a) {
     for (int e = 0; e < PT; ++e) y[e] += parts[x * WS + row * OROW + d0 + e] * f;
   }
   if (whole) {
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     const int rr = 16 * block + row;
+    const float inv = ka_inverse(a, sum, jb, jlen - (a.L - 1 - rr / a.group));
     uint16_t* out = a.out + jb * a.out_strides[0] + (int64_t)(rr / a.group) * a.out_strides[1] +
                     (int64_t)(h * a.group + rr % a.group) * a.out_strides[2] + d0;
 #pragma unroll
@@ -545,7 +561,7 @@ __global__ __launch_bounds__(256) void attention_kv4_join_kernel(Kv4AttnArgs a) 
   const int i = (int)(rest - (uint32_t)b * (uint32_t)a.L);
   const int HB = a.c.heads * a.blocks, h = hq / a.group, r = i * a.group + hq % a.group;
   const KaLens lens(a, lane);
-  const int nt = ka_tiles(lens.keys(a, b));
+  const int len = lens.keys(a, b), nt = ka_tiles(len);
   const int s0 = lens.before(a, b, lane) * HB + (h * a.blocks + r / 16) * nt, s1 = s0 + nt;
   const int all = lens.all * HB;
   const int W0 = ka_wave_of(s0, all), W1 = ka_wave_of(s1 - 1, all);
@@ -607,7 +623,7 @@ __global__ __launch_bounds__(256) void attention_kv4_join_kernel(Kv4AttnArgs a) 
 #pragma unroll
     for (int x = 1; x < NW; ++x) y += *reinterpret_cast<const vec*>(&red[x][lane * PER]);
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const float inv = ka_inverse(a, sum, b, len - (a.L - 1 - i));
   uint16_t* out = a.out + b * a.out_strides[0] + (int64_t)i * a.out_strides[1] + (int64_t)hq * a.out_strides[2];
 #pragma unroll
   for (int e = 0; e < PER; ++e) out[lane * PER + e] = (uint16_t)f32_to_bf16(y[e] * inv);

@@ -451,8 +451,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_packed_kernel(PackedArgs
 
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
+    // No key seen: zeros; only scores of -infinity: NaN.
     const float l = quad_sum(lsum[rb]);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = l == 0.f && lim[rb] < 0 ? 0.f : 1.0f / l;
     const int r = 32 * w + 16 * rb + l16;
     if (r >= left) continue;
     const int rr = rbase + r;

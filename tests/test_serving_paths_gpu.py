@@ -82,3 +82,66 @@ def test_attention_kv4_largest_values(D):
     ref, mag = serving.attention(q, kq, vq, 1.0, np.ones((1, n), bool))
     bound = _attention_bound(ref, mag, q, k, 1.0, n, kv4=True)
     _check(got, np.tile(ref, (B, 1, 1, 1)), np.tile(bound, (B, 1, 1, 1)), f"kv4 largest values {D}")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D,tail", [(64, 0), (128, 0), (64, 8200), (128, 8200)])
+def test_attention_packed_scores_of_minus_infinity(D, tail, causal):
+    """A query that sees keys, but only with the score -infinity, has no softmax:
+    NaN, where one that sees no key gives zeros.  One that sees another key
+    too has that one's value."""
+    ops = _ops()
+    rng = np.random.default_rng(4)
+    nq, nk = 70, 50 + tail  # causal: the first 20 queries see nothing where tail = 0
+    q = np.zeros((nq, 1, D), np.float32)
+    q[:, 0, 0] = 1.0
+    k = np.zeros((nk, 1, D), np.float32)
+    k[:, 0, 0] = -np.inf
+    v = _rand(rng, (nk, 1, D))
+
+    def run():
+        return _down(ops.attention_packed(_up(q), _up(k), _up(v), _cu([nq]), 1.0, cu_seqlens_k=_cu([nk]),
+                                          causal=causal))[:, 0]
+
+    last = np.arange(nq) + nk - nq if causal else np.full(nq, nk - 1)
+    got = run()
+    assert (got[last < 0] == 0).all() and np.isnan(got[last >= 0]).all()
+    one = nk - 30
+    k[one] = 0.0
+    got = run()
+    assert (got[last < 0] == 0).all() and np.isnan(got[(last >= 0) & (last < one)]).all()
+    assert np.array_equal(got[last >= one], np.repeat(v[one].astype(np.float64), (last >= one).sum(), 0))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,B,H", [(30, 4, 2), (250, 4, 4), (1000, 4, 2), (200, 70, 8)])
+def test_attention_kv4_scores_of_minus_infinity(n, B, H, D):
+    """The same over the cache, where scores pass the f32 range: q . k is
+    -10^30 times up to 10^30.  Keys in pages the cache does not have are not
+    seen."""
+    ops = _ops()
+    page = 16
+    rng = np.random.default_rng(5)
+    q = np.zeros((B, 2, H, D), np.float32)
+    q[..., 0] = 2.0 ** 100
+    k = np.zeros((n, H, D), np.float32)
+    k[:, :, 0] = -2.0 ** 100
+    v = _rand(rng, (n, H, D))
+    pages = -(-n // page)
+    cache = ops.KV4Cache(pages, H, page, D, device=DEV)
+    table = np.tile(np.arange(pages), (B, 1))
+    table[1] = -1                     # no page: zeros
+    table[2, 1:] = pages + 1          # the first page alone
+
+    def run():
+        ops.kv4_append(cache, _up(k), _up(v), _ints(np.arange(n), torch.int64))
+        return _down(ops.attention_kv4(_up(q), cache, _ints(table), _ints([1] + [n] * (B - 1)), 1.0))
+
+    got = run()
+    assert (got[0, 0] == 0).all() and np.isnan(got[0, 1]).all()  # one key: the last query alone sees it
+    assert (got[1] == 0).all() and np.isnan(got[2:]).all()
+    k[n - 1] = 0.0
+    got = run()
+    vn = serving.kv4_values(*serving.kv4(v[n - 1]))
+    assert (got[1] == 0).all() and np.isnan(got[2]).all() and np.isnan(got[3:, 0]).all()
+    assert np.array_equal(got[3:, 1], np.tile(round_bf16(vn.astype(np.float32)).astype(np.float64), (max(B - 3, 0), 1, 1)))
