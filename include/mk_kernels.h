@@ -404,9 +404,10 @@ int mk_merge_heads_bf16(const void* o, void* out, int64_t B, int64_t H, int64_t 
  *   c, s from row positions[t] of cos_table / sin_table f32 [table_len, R/2];
  *   pair i is dimensions (i, i + R/2) (MK_ROPE_HALF) or (2i, 2i + 1)
  *   (MK_ROPE_INTERLEAVED).  f32 inside, one rounding.  strides: token and head
- *   stride of q, k, q_out, k_out.  The outputs may be the inputs.  A negative
- *   position marks padding, its rows are not written; a position of table_len
- *   or more gives NaN.  D % 8 == 0, D <= 512, R % 8 == 0, R <= D; heads and gains
+ *   stride of q, k, q_out, k_out.  q_out may be q, k_out may be k.  A negative
+ *   position marks padding: its rows are not written, or, with MK_ROPE_CLEAR_Q
+ *   (MK_ROPE_CLEAR_K) added to the layout, are zeros in q_out (k_out).  A position
+ *   of table_len or more gives NaN.  D % 8 == 0, D <= 512, R % 8 == 0, R <= D; heads and gains
  *   aligned to 4 elements, tables to 16 bytes.
  *
  * mk_kv4_cache: keys and values in 4 bits.  A group of 64 dimensions of one
@@ -457,7 +458,7 @@ int mk_merge_heads_bf16(const void* o, void* out, int64_t B, int64_t H, int64_t 
  * times the scale, p below 2^-5, is rounded to bf16).  scale must be positive
  * and finite.
  * ---------------------------------------------------------------------- */
-enum { MK_ROPE_HALF = 0, MK_ROPE_INTERLEAVED = 1 };
+enum { MK_ROPE_HALF = 0, MK_ROPE_INTERLEAVED = 1, MK_ROPE_CLEAR_Q = 0x100, MK_ROPE_CLEAR_K = 0x200 };
 
 int mk_qk_norm_rope(int dtype, const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides,
                     const int32_t* positions, const float* cos_table, const float* sin_table, int64_t table_len,

@@ -36,6 +36,7 @@ struct RotateArgs {
   int Hq, H;     // query heads, query and key heads
   int D, R;
   float eps;
+  bool clear[2];  // padding rows are zeros, else left as they were
 };
 
 // 4 elements of a lane as they are in memory.
@@ -113,7 +114,18 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RotateArgs a) {
       hi[i] = *reinterpret_cast<const RotRun<E>*>(src + off1);
     }
   }
-  if (pos < 0) return;  // padding: the row is left as it was
+  if (pos < 0) {  // padding
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int h = first + 4 * i * HPW, part = h < a.Hq ? 0 : 1;
+      if (!mine[i] || !a.clear[part]) continue;
+      const float zeros[8] = {};
+      E* dst = static_cast<E*>(a.out[part]) + t * a.out_tok[part] + (h - (part ? a.Hq : 0)) * a.out_head[part];
+      rot_store(dst + off0, zeros, 0);
+      rot_store(dst + off1, zeros, 4);
+    }
+    return;
+  }
   const bool known = pos < a.table_len;
   f32x4 cv = {1.f, 1.f, 1.f, 1.f}, sv = {0.f, 0.f, 0.f, 0.f};
   if (turn && known) {
@@ -207,6 +219,8 @@ extern "C" int mk_qk_norm_rope(int dtype, const void* q, const void* k, void* q_
   mkc::clear_error();
   const char* fn = "mk_qk_norm_rope";
   if (dtype != MK_DT_F32 && dtype != MK_DT_BF16) return mkc::fail(MK_EUNSUPPORTED, "%s: dtype %d", fn, dtype);
+  const int flags = layout & (MK_ROPE_CLEAR_Q | MK_ROPE_CLEAR_K);
+  layout -= flags;
   if (layout != MK_ROPE_HALF && layout != MK_ROPE_INTERLEAVED)
     return mkc::fail(MK_EINVAL, "%s: layout %d", fn, layout);
   if (T < 0 || Hq < 0 || Hkv < 0 || Hq + Hkv <= 0 || D <= 0 || R < 0 || table_len < 0)
@@ -254,6 +268,8 @@ extern "C" int mk_qk_norm_rope(int dtype, const void* q, const void* k, void* q_
   a.D = (int)D;
   a.R = (int)R;
   a.eps = eps;
+  a.clear[0] = flags & MK_ROPE_CLEAR_Q;
+  a.clear[1] = flags & MK_ROPE_CLEAR_K;
   int lpr = 8;
   while (8 * lpr < D) lpr *= 2;
   const int groups = (a.H * lpr + 63) / 64;

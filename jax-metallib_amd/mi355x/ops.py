@@ -581,7 +581,8 @@ def qk_norm_rope(q, k, positions, cos_table, sin_table, g_q=None, g_k=None, eps=
     "half" pairs dimension i with i + R/2, "interleaved" 2i with 2i + 1.
     q_out = q and k_out = k work in place.  Every head starts at a multiple of
     4 elements, D and R are multiples of 8.  Rows with a negative position are
-    not written; a position that the tables do not hold gives NaN."""
+    left as they were in a given output and zeros in one made here; a position
+    that the tables do not hold gives NaN."""
     T, Hq, D = shape = q.shape
     dev, dt = q.device, q.dtype
     sq = _strides(q, "q", _F32_BF16, shape, dev)
@@ -594,7 +595,9 @@ def qk_norm_rope(q, k, positions, cos_table, sin_table, g_q=None, g_k=None, eps=
         _index(g_q, "g_q", dt, (D,), dev)
     if g_k is not None:
         _index(g_k, "g_k", dt, (D,), dev)
+    flags = 0
     if q_out is None:
+        flags = _lib.MK_ROPE_CLEAR_Q
         q_out = torch.empty_like(q)
         so = q_out.stride()
     else:
@@ -605,6 +608,7 @@ def qk_norm_rope(q, k, positions, cos_table, sin_table, g_q=None, g_k=None, eps=
         kshape = (T, Hkv, D)
         sk = _strides(k, "k", types, kshape, dev)
         if k_out is None:
+            flags |= _lib.MK_ROPE_CLEAR_K
             k_out = torch.empty_like(k)
             sko = k_out.stride()
         else:
@@ -618,7 +622,7 @@ def qk_norm_rope(q, k, positions, cos_table, sin_table, g_q=None, g_k=None, eps=
     _launch(dev, lambda stream: lib().mk_qk_norm_rope(
         code, q.data_ptr(), _ptr(k), q_out.data_ptr(), _ptr(k_out), strides, positions.data_ptr(),
         cos_table.data_ptr(), sin_table.data_ptr(), length, _ptr(g_q), _ptr(g_k), eps, T, Hq, Hkv, D, 2 * R2,
-        _ROPE_LAYOUTS[layout], stream))
+        _ROPE_LAYOUTS[layout] | flags, stream))
     return q_out, k_out
 
 

@@ -145,3 +145,30 @@ def test_attention_kv4_scores_of_minus_infinity(n, B, H, D):
     vn = serving.kv4_values(*serving.kv4(v[n - 1]))
     assert (got[1] == 0).all() and np.isnan(got[2]).all() and np.isnan(got[3:, 0]).all()
     assert np.array_equal(got[3:, 1], np.tile(round_bf16(vn.astype(np.float32)).astype(np.float64), (max(B - 3, 0), 1, 1)))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,Hq,Hkv,D,layout", [(5, 2, 1, 64, "half"), (3, 20, 20, 80, "interleaved"),
+                                               (1100, 32, 8, 128, "half")])
+def test_qk_norm_rope_padding_of_new_outputs_is_zero(T, Hq, Hkv, D, layout, dt):
+    """Rows with a negative position: zeros in an output made here, left as
+    they were in one that is given, also where only one of the two is."""
+    ops = _ops()
+    rng = np.random.default_rng(T)
+    q, k = _up(_rand(rng, (T, Hq, D)), dt), _up(_rand(rng, (T, Hkv, D)), dt)
+    pos = rng.integers(0, 9, T)
+    pos[[1, T - 1]] = [-1, -2 ** 31]
+    kept = torch.from_numpy(pos >= 0).to(DEV)
+    cos, sin = ops.rope_tables(9, 32, device=DEV)
+    given = [torch.full_like(t, 7.0) for t in (q, k)]
+    ops.qk_norm_rope(q, k, _ints(pos), cos, sin, layout=layout, q_out=given[0], k_out=given[1])
+    for outs in ({}, {"q_out": 0}, {"k_out": 1}):
+        dirty = [torch.full_like(t, float("nan")) for t in (q, k)]  # what an allocator may hand out again
+        del dirty
+        kw = {name: torch.full_like((q, k)[i], 7.0) for name, i in outs.items()}
+        y = ops.qk_norm_rope(q, k, _ints(pos), cos, sin, layout=layout, **kw)
+        for got, want, name in zip(y, given, ("q_out", "k_out")):
+            assert torch.equal(got[kept], want[kept])
+            assert (got[~kept] == (7.0 if name in kw else 0.0)).all()
+    alone, none = ops.qk_norm_rope(q, None, _ints(pos), cos, sin, layout=layout)
+    assert none is None and (alone[~kept] == 0).all() and torch.equal(alone[kept], given[0][kept])
