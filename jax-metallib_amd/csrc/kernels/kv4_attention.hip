@@ -646,11 +646,12 @@ int64_t kv4_most_tiles(int64_t B, int64_t L, int64_t Hq, int64_t Hkv, int64_t wi
   return items * (tiles > 0 ? tiles : 1);
 }
 
-// Sizes both entry points take.
+// Sizes both entry points take (those of the cache as kv4_view has them).
 bool kv4_sizes_ok(int64_t B, int64_t L, int64_t Hq, int64_t Hkv, int64_t width, int64_t page) {
-  return B >= 0 && B <= 65536 && L > 0 && L <= (1 << 20) && Hq > 0 && Hq <= 65536 && Hkv > 0 && Hq % Hkv == 0 &&
-         B * L <= (int64_t)1 << 30 && B * L * Hq < (int64_t)1 << 24 && width >= 0 && width <= (int64_t)1 << 28 &&
-         page > 0 && width * page <= (int64_t)1 << 28 && kv4_most_tiles(B, L, Hq, Hkv, width, page) < (int64_t)1 << 31;
+  return B >= 0 && B <= 65536 && L > 0 && L <= (1 << 20) && Hq > 0 && Hq <= 65536 && Hkv > 0 && Hkv <= 65535 &&
+         Hq % Hkv == 0 && B * L <= (int64_t)1 << 30 && B * L * Hq < (int64_t)1 << 24 && width >= 0 &&
+         width <= (int64_t)1 << 28 && page > 0 && page % 16 == 0 && page <= 1024 &&
+         width * page <= (int64_t)1 << 28 && kv4_most_tiles(B, L, Hq, Hkv, width, page) < (int64_t)1 << 31;
 }
 
 // Workgroups that take a share of at most `most` tiles.

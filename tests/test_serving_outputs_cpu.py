@@ -71,3 +71,15 @@ def test_exactly_the_overlapping_layouts_are_refused():
     far = i64s(*[1 << 40, 1 << 39] * 4)
     assert b"scale" in _last(_packed(Tq=2, Tk=2, Hq=2, Hkv=2, scale=3e38, strides=far))
     assert SHARE in _last(_packed(Tq=1 << 27, Tk=1 << 27, Hq=4, Hkv=4, scale=3e38, strides=far))
+
+
+def test_kv4_workspace_query_refuses_what_the_call_refuses():
+    """-1 for every size that the attention itself refuses, also where a
+    product of sizes would pass 64 bits."""
+    need = _lib.lib().mk_attention_kv4_workspace_bytes
+    assert need(1, 1, 65535, 65535, 64, 4, 1024) > 0
+    for bad in ((2, 1, 4, 2, 64, 1 << 24, 1 << 40), (2, 1, 4, 2, 64, 4, 1 << 62), (2, 1, 4, 2, 64, 4, 24),
+                (2, 1, 4, 2, 64, 4, 8), (2, 1, 4, 2, 64, 4, 2048), (1, 1, 65536, 65536, 64, 4, 16)):
+        assert need(*bad) == -1, bad
+    for page, heads in ((24, 2), (2048, 2), (16, 65536)):
+        assert _kv4_attention(cache=_cache(page=page, heads=heads), Hq=heads, B=1) != _lib.MK_OK
