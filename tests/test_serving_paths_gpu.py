@@ -11,7 +11,7 @@ import pytest
 from _gpu import torch
 from oracle import serving
 from oracle.bf16 import round_bf16
-from test_serving_ops_gpu import DEV, _attention_bound, _check, _cu, _down, _ints, _ops, _rand, _up
+from test_serving_ops_gpu import DEV, _attention_bound, _check, _cu, _down, _ints, _ops, _rand, _rotate_bound, _up
 
 pytestmark = pytest.mark.gpu
 
@@ -172,3 +172,51 @@ def test_qk_norm_rope_padding_of_new_outputs_is_zero(T, Hq, Hkv, D, layout, dt):
             assert (got[~kept] == (7.0 if name in kw else 0.0)).all()
     alone, none = ops.qk_norm_rope(q, None, _ints(pos), cos, sin, layout=layout)
     assert none is None and (alone[~kept] == 0).all() and torch.equal(alone[kept], given[0][kept])
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("T,Hq,Hkv,D,R,norm", [
+    (1024, 32, 8, 128, 128, True), (1025, 21, 3, 128, 64, True), (1100, 7, 14, 256, 64, True), (1030, 3, 2, 512, 512, True),
+    (1024, 32, 9, 64, 40, False), (1500, 40, 1, 80, 80, True), (1024, 5, 0, 512, 8, True), (1300, 33, 32, 8, 8, True)])
+def test_qk_norm_rope_of_many_tokens(T, Hq, Hkv, D, R, norm, layout, dt):
+    """From 1024 tokens and more than 4 groups of heads on, a wave takes three
+    groups, the last ones of a token in part: against float64, bit for bit the
+    calls of fewer tokens, and in place with padding and unknown positions."""
+    ops = _ops()
+    rng = np.random.default_rng(T + Hq + D)
+    lanes = max(8, 1 << (D // 8 - 1).bit_length())
+    assert -(-(Hq + Hkv) * lanes // 64) > 4  # groups of heads that a wave holds at once
+    qkv = _rand(rng, (T, Hq + 2 * Hkv, D), 1.5)
+    gains = [round_bf16(rng.uniform(0.5, 1.5, D).astype(np.float32)) if norm else None for _ in range(2)]
+    pos = rng.integers(0, 77, T)
+    cos, sin = ops.rope_tables(77, R, device=DEV)
+    x = _up(qkv, dt)
+    g = [None if a is None else _up(a, dt) for a in gains]
+    g[1] = g[1] if Hkv else None
+
+    def run(lo, hi, at, **kw):
+        k = x[lo:hi, Hq:Hq + Hkv] if Hkv else None
+        return ops.qk_norm_rope(x[lo:hi, :Hq], k, _ints(at[lo:hi]), cos, sin, g_q=g[0], g_k=g[1], layout=layout, **kw)
+
+    whole = run(0, T, pos)
+    parts = [run(0, 700, pos), run(700, T, pos)]
+    c, s = cos.double().cpu().numpy()[pos], sin.double().cpu().numpy()[pos]
+    for i, (heads, gain) in enumerate(((slice(0, Hq), gains[0]), (slice(Hq, Hq + Hkv), gains[1]))):
+        if i and not Hkv:
+            assert whole[1] is None
+            continue
+        assert torch.equal(whole[i], torch.cat([p[i] for p in parts]))
+        ref = serving.rotate(qkv[:, heads], gain, c, s, layout, 1e-6)
+        _check(_down(whole[i]), ref, _rotate_bound(qkv[:, heads], ref, norm, D, dt), f"rotate {T}x{D} R{R} {layout}")
+    # In place, with rows that are left and rows of no position.
+    at = pos.copy()
+    at[::17], at[5::23] = -1, 77
+    kept, lost = torch.from_numpy(at < 0).to(DEV), torch.from_numpy(at == 77).to(DEV)
+    known = ~(kept | lost)
+    before = x.clone()
+    run(0, T, at, q_out=x[:, :Hq], **({"k_out": x[:, Hq:Hq + Hkv]} if Hkv else {}))
+    turned = x[:, :Hq + Hkv]
+    want = torch.cat([w for w in whole if w is not None], 1)
+    assert torch.equal(turned[known], want[known]) and torch.equal(turned[kept], before[kept][:, :Hq + Hkv])
+    assert torch.isnan(turned[lost]).all() and torch.equal(x[:, Hq + Hkv:], before[:, Hq + Hkv:])
