@@ -11,7 +11,8 @@ import pytest
 from _gpu import torch
 from oracle import serving
 from oracle.bf16 import round_bf16
-from test_serving_ops_gpu import DEV, _attention_bound, _check, _cu, _down, _ints, _ops, _rand, _rotate_bound, _up
+from test_serving_ops_gpu import (DEV, _attention_bound, _check, _cu, _down, _ints, _kv4_case, _ops, _rand,
+                                  _rotate_bound, _up)
 
 pytestmark = pytest.mark.gpu
 
@@ -220,3 +221,56 @@ def test_qk_norm_rope_of_many_tokens(T, Hq, Hkv, D, R, norm, layout, dt):
     want = torch.cat([w for w in whole if w is not None], 1)
     assert torch.equal(turned[known], want[known]) and torch.equal(turned[kept], before[kept][:, :Hq + Hkv])
     assert torch.isnan(turned[lost]).all() and torch.equal(x[:, Hq + Hkv:], before[:, Hq + Hkv:])
+
+
+@pytest.mark.parametrize("lens,L,Hq,Hkv,D", [
+    ([1, 63, 200], 1, 8, 2, 128), ([300, 700], 5, 16, 2, 64), ([400] * 96, 2, 16, 8, 64), ([130, 5] * 300, 1, 32, 8, 128)])
+def test_attention_kv4_over_its_queries(lens, L, Hq, Hkv, D):
+    """out = q, also as a view: the bits of a call with an output of its own,
+    with items of one wave, of one workgroup and of several."""
+    ops = _ops()
+    q, _, _, cache, table = _kv4_case(ops, lens, L, Hq, Hkv, D, 64, 3)
+    B, t, n = len(lens), _ints(table), _ints(lens)
+    want = ops.attention_kv4(_up(q), cache, t, n, 0.1)
+    x = torch.full((B, L, Hq + 3, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    for rest in (x, x.transpose(0, 1).contiguous().transpose(0, 1)):
+        rest[:, :, :Hq] = _up(q)
+        view = rest[:, :, :Hq]
+        y = ops.attention_kv4(view, cache, t, n, 0.1, out=view)
+        assert y is view and torch.equal(rest[:, :, :Hq], want) and (rest[:, :, Hq:] == 7.0).all()
+
+
+def test_far_slots():
+    """Slots from 2^30 on with pages of 1024, where the page is found by a
+    division: the numbers of near slots, on both sides of that place."""
+    ops = _ops()
+    page, edge = 1024, 2 ** 30
+    rng = np.random.default_rng(6)
+    slots = np.concatenate([[0, 1023, 1024], edge + np.array([-1025, -1024, -1, 0, 1, 1023, 1024, 2047])])
+    T = len(slots)
+    k, v = _up(_rand(rng, (T, 1, 64))), _up(_rand(rng, (T, 1, 64)))
+    near = ops.KV4Cache(1, 1, 16, 64, device=DEV)
+    ops.kv4_append(near, k, v, _ints(np.arange(T), torch.int64))
+    want = ops.kv4_read(near, _ints(np.arange(T), torch.int64), dtype=torch.float32)
+    far = ops.KV4Cache(edge // page + 2, 1, page, 64, device=DEV)  # 75 GB
+    at = _ints(slots, torch.int64)
+    ops.kv4_append(far, k, v, at)
+    for got, w in zip(ops.kv4_read(far, at, dtype=torch.float32), want):
+        assert torch.equal(got, w)
+    # In the places that the format documents.
+    for a, b in zip((far.k_scale, far.v_scale, far.k_zero, far.v_zero),
+                    (near.k_scale, near.v_scale, near.k_zero, near.v_zero)):
+        assert torch.equal(a[at // page, 0, 0, at % page], b[0, 0, 0, :T])
+    empty = torch.cat([at[3:] - 3, at[3:] + 5])
+    empty = empty[~torch.isin(empty, at) & (empty < far.pages * page)]
+    assert all((t == 0).all() for t in ops.kv4_read(far, empty))
+    # Attention over the last page reads the same keys.
+    q = _up(_rand(rng, (1, 1, 1, 64)))
+    last = _ints([[edge // page + 1]])
+    alone = ops.KV4Cache(1, 1, page, 64, device=DEV)
+    for name in ("k", "k_scale", "k_zero", "v", "v_scale", "v_zero"):
+        getattr(alone, name)[0] = getattr(far, name)[edge // page + 1]
+    y = ops.attention_kv4(q, far, last, _ints([page]), 0.1)
+    assert torch.equal(y, ops.attention_kv4(q, alone, _ints([[0]]), _ints([page]), 0.1)) and (y != 0).any()
+    del far
+    torch.cuda.empty_cache()
