@@ -13,9 +13,11 @@
 // an infinity reads back as NaN.
 //
 // Layout: a lane holds 8 dimensions (16 bytes in, one dword out) of the key and
-// of the value, a group is 8 lanes.  Both directions are one pass bound by HBM:
-// 8000 tokens of 8 heads of 128 in 12.0 us (3.4 TB/s) and back in 8.4 (5.0);
-// the way in issues 374 vector instructions a wave, 4 keys and values (counted).
+// of the value, a group is 8 lanes.  Both directions are one pass.  8000 tokens
+// of 8 heads of 128 (in a graph): in 11.3 us (3.7 TB/s), bound by its 374 vector
+// instructions a wave, 4 keys and values (counted: 9.7 us of issue); back to bf16
+// in 7.8 (5.4 TB/s, partly from the cache), to f32 in 37 (2.0 TB/s; each lane's
+// 32 bytes go out in two stores).
 #include "kv4.h"
 
 namespace mk {
@@ -134,8 +136,8 @@ __device__ __forceinline__ uint32_t kv4_quantise(const u32x4& xw, uint32_t* scal
 // The row (token, head) of a thread: D / 8 threads a row, a workgroup 16 tokens
 // of one head (two of 64 dimensions), so that neighbouring rows are neighbours
 // in a page and their scales and zero points share lines (8000 tokens of 8
-// heads in and out: 20.8 us, against 21.6 with the heads of a token one after
-// the other).
+// heads in and out, when this was chosen: 20.8 us, against 21.6 with the heads of
+// a token one after the other; 18.6 since places and scales are multiplications).
 template <int D>
 __device__ __forceinline__ bool kv4_row(const Kv4Rows& a, uint32_t* t, uint32_t* h) {
   const uint32_t row = threadIdx.x / (D / 8);

@@ -16,8 +16,12 @@
 //     an XOR-swizzled LDS tile), second the wave's Q rows (registers): a lane
 //     holds row l%16 and the keys 4(l/16) .. +3 of each 16.
 //   O += V^T P^T: second operand P straight from those registers, rounded to
-//     bf16 as the matrix cores need (the sum l takes the unrounded p); the V
-//     fragment is read transposed from the rows of the same keys.
+//     bf16 (the sum l takes the unrounded p); the V fragment is read transposed
+//     from the rows of the same keys.  Both operands of a matrix instruction have
+//     one type, and v needs the range of bf16; p in two parts would keep its
+//     bits at twice the products of this half.  The rounding is half a step,
+//     2^-8 of each term: against 64 bits the results are off by 0.0019 .. 0.0023
+//     of their size, where rounding the result alone gives 0.0015 .. 0.0017.
 // Matrix and vector work must overlap, which the two waves of a SIMD do for each
 // other:
 //   8 waves: two groups of 4, one wave of each on every SIMD.  A tile is two
@@ -29,9 +33,12 @@
 //     softmax at raised priority); two stages, one tile ahead.  Each one's
 //     start and end lie under the other's work.
 // Bound by the matrix cores and the exponentials together, one exponential for
-// 4 D operations: 6097 queries of 32 heads over 24385 keys of 8 take 1.16 ms,
-// 1.02 PFLOP/s where a large product reaches 1.2.  Short prompts pay for the
-// queries' loads, the first tiles and the stores around few tiles.
+// 4 D operations: 6097 queries of 32 heads over 24385 keys of 8 take 1.14 ms (in
+// a graph), 1.05 PFLOP/s where a large product reaches 1.2.  Short prompts pay for
+// the queries' loads, the first tiles and the stores around few tiles; few queries
+// behind long keys for a workgroup's walk over all of them (64 of 32 heads behind
+// 8192: 249 us).  With D = 128 the second pass spills 8 (4 waves: 12) registers;
+// the first, which all rows take, none.
 #include "wave.h"
 
 #include <math.h>
@@ -542,7 +549,11 @@ extern "C" int mk_attention_packed_bf16(const void* q, const void* k, const void
   // 8 waves and phases where sequences are long (one of 8192 keys: 568 against
   // 585 us with 4 waves, 6097 queries over 24385 keys 1177 / 1230), 4 waves and
   // two workgroups per CU elsewhere (16 of 1024: 219 / 231 us, 8 ragged ones of
-  // 64 .. 2100: 157 / 166, 4 of 1 .. 300: 13.1 / 17.7; even at 4096).
+  // 64 .. 2100: 157 / 166, 4 of 1 .. 300: 13.1 / 17.7; even at 4096).  The rule
+  // takes the mean length, keys behind the last sequence included.  With few
+  // queries behind long keys either can win (8192 keys, 8 / 4 waves: 1 query 189
+  // / 217 us, 64 249 / 222, 1024 252 / 224, 64 in each of 8 sequences 264 / 275),
+  // and one long prompt among short ones has 4 (8192 and seven of 1: 561 / 575).
   const bool big = Tk / B >= 4096;
   const int64_t tiles = Tq * a.group / (big ? 256 : 128) + B;
   if (!mkc::grid_fits(tiles * Hkv, big ? 512 : 256)) return mkc::fail(MK_EINVAL, "%s: shape too large", fn);

@@ -17,7 +17,7 @@
 // per row) heads of one token at a time, and the norm is a sum over those
 // lanes by row shifts.  A workgroup is 4 waves of one token, each with U
 // groups of heads whose loads are all in flight before the first is used.
-// Bound by HBM with many tokens (8191 of 40 heads, 169 MB: 38.7 us, 4.4 TB/s),
+// Bound by HBM with many tokens (8191 of 40 heads, 169 MB: 38.5 us, 4.4 TB/s),
 // by launch and two dependent loads (position, then table row) with few.
 #include "wave.h"
 
@@ -56,7 +56,9 @@ struct RotRun<uint16_t> {
 };
 
 // The outputs are not read here again: stored past the L2's lines in use (8191
-// tokens of 40 heads: 38.7 us, against 43.7 with plain stores).
+// tokens of 40 heads: 38.7 us, against 43.7 with plain stores).  What reads them
+// next loses by it what this gains, no more: rotation in place, cache and packed
+// attention of 8191 tokens take 169.5 us either way, of 500 29.9.
 __device__ __forceinline__ void rot_store(float* p, const float (&f)[8], int i) {
   __builtin_nontemporal_store(f32x4{f[i], f[i + 1], f[i + 2], f[i + 3]}, reinterpret_cast<f32x4*>(p));
 }
