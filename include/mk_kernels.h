@@ -391,8 +391,9 @@ int mk_merge_heads_bf16(const void* o, void* out, int64_t B, int64_t H, int64_t 
  * benchmarks/vs_cpu.py:603-626, has whole sequences of one length and no
  * cache).  Strides are in elements, must be >= 0 and keep every head's start
  * aligned as stated; dimensions within a head are contiguous, and an output's
- * heads must not share memory (MK_EINVAL).  Values that
- * live in device memory (positions, slots, block table entries, lengths,
+ * heads must not share memory (MK_EINVAL; nor must two outputs of a call, or an
+ * output and an input but where a call says so: this is not checked).  Values
+ * that live in device memory (positions, slots, block table entries, lengths,
  * offsets) are checked by the kernels, which never read or write outside the
  * sizes given: what a wrong value gives is stated per call.
  *
@@ -407,8 +408,8 @@ int mk_merge_heads_bf16(const void* o, void* out, int64_t B, int64_t H, int64_t 
  *   stride of q, k, q_out, k_out.  q_out may be q, k_out may be k.  A negative
  *   position marks padding: its rows are not written, or, with MK_ROPE_CLEAR_Q
  *   (MK_ROPE_CLEAR_K) added to the layout, are zeros in q_out (k_out).  A position
- *   of table_len or more gives NaN.  D % 8 == 0, D <= 512, R % 8 == 0, R <= D; heads and gains
- *   aligned to 4 elements, tables to 16 bytes.
+ *   of table_len or more gives NaN.  D % 8 == 0, D <= 512, R % 8 == 0, R <= D;
+ *   heads and gains aligned to 4 elements, tables to 16 bytes.
  *
  * mk_kv4_cache: keys and values in 4 bits.  A group of 64 dimensions of one
  *   token and head has a bf16 scale s and a zero point z in 0 .. 15, its

@@ -274,3 +274,25 @@ def test_far_slots():
     assert torch.equal(y, ops.attention_kv4(q, alone, _ints([[0]]), _ints([page]), 0.1)) and (y != 0).any()
     del far
     torch.cuda.empty_cache()
+
+
+def test_expanded_inputs():
+    """Inputs whose tokens or heads are one (strides of 0), as expand makes
+    them: the bits of the copies."""
+    ops = _ops()
+    rng = np.random.default_rng(10)
+    T, Hq, Hkv, D = 37, 4, 2, 64
+    cos, sin = ops.rope_tables(T, D, device=DEV)
+    pos, cu, slots = _ints(np.arange(T)), _cu([20, 17]), _ints(np.arange(T), torch.int64)
+    table, lens = _ints(np.tile(np.arange(3), (2, 1))), _ints([37, 20])
+    for one in ((1, Hq, D), (T, 1, D), (1, 1, D)):
+        q = _up(_rand(rng, one)).expand(T, Hq, D)
+        k = _up(_rand(rng, (one[0], min(one[1], Hkv), D))).expand(T, Hkv, D)
+        got = []
+        for a, b in ((q, k), (q.contiguous(), k.contiguous())):
+            cache = ops.KV4Cache(3, Hkv, 16, D, device=DEV)
+            ops.kv4_append(cache, b, b, slots)
+            got.append([*ops.qk_norm_rope(a, b, pos, cos, sin), *ops.kv4_read(cache, slots),
+                        ops.attention_packed(a, b, b, cu, 0.1),
+                        ops.attention_kv4(a[:2].unsqueeze(1), cache, table, lens, 0.1)])
+        assert all(torch.equal(x, y) for x, y in zip(*got))
